@@ -196,10 +196,10 @@ __global__ void __launch_bounds__(kThreads) m1_conv_bwd_kernel(ConvBwdParams p, 
         x += s0 - lead;
         dout += s0 - lead;
         dx += s0 - lead;
-        // a lane's elements in the row: from `head` on in the row's first iteration,
-        // up to `tail` in its last
+        // a lane's elements in the row: from `head` on in the row's first iteration (which
+        // is iteration 0 of its first split only), up to `tail` in its last
         const bool has_first = begin == 0 && lead > 0;
-        const int head = max(0, lead - lane * kE);
+        const int head = has_first ? max(0, lead - lane * kE) : 0;
         const int tail = static_cast<int>(max(static_cast<int64_t>(0), min(lead + p.len - s0, static_cast<int64_t>(kE))));
         const bool cut = lead + p.len - s0 + lane * kE < kRun;  // the last iteration holds the row's end
         // Iteration `it` (its first element `back` before the last iteration's).

@@ -1,0 +1,54 @@
+"""Training-step calls as programs make them: tensors off their boundaries, tracing and mapping,
+mixed devices, autocast, gradients that are kept.
+
+Tolerances are those of test_training_gpu.py, derived there; comparisons of two calls that run the
+same kernels on the same values are bitwise.
+"""
+
+import pytest
+import torch
+
+from test_training_gpu import BF16_TOL, TOL, conv_reference, gen, rel
+
+pytestmark = pytest.mark.gpu
+
+
+def arm():
+    import armhackathon_b200 as a
+    return a
+
+
+# ---------------------------------------------------------------------------
+# causal conv1d + SiLU
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,dim,length", [(1, 3, 5000), (2, 2, 4097), (1, 1, 700)])
+@pytest.mark.parametrize("kernel", [4, 8])
+def test_conv_backward_of_tensors_that_lie_alike_off_a_boundary(batch, dim, length, kernel, dtype):
+    # x, dout and dx start the same number of elements past a 16-byte boundary, and few rows are
+    # split in time: the C entry sets no rule for where they start
+    from armhackathon_b200 import _ffi
+    g = gen(length)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    w, bias = r(dim, kernel), r(dim)
+    n, code = batch * dim * length, {torch.float32: 0, torch.bfloat16: 1}[dtype]
+    for off in range(1, 4 if dtype == torch.float32 else 8):
+        x, dout, dx = (r(n + 16).to(dtype) for _ in range(3))
+        guard = dx.clone()
+        cut = lambda t: t[off:off + n].view(batch, dim, length)  # noqa: E731
+        dw, db = torch.empty_like(w), torch.empty_like(bias)
+        nbytes = _ffi.conv_silu_backward_workspace_bytes(batch, dim, length, kernel)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        _ffi.conv_silu_backward_raw(batch, dim, length, kernel, code, cut(dout).data_ptr(),
+                                    cut(x).data_ptr(), w.data_ptr(), bias.data_ptr(), ws.data_ptr(),
+                                    nbytes, cut(dx).data_ptr(), dw.data_ptr(), db.data_ptr(),
+                                    torch.cuda.current_stream().cuda_stream)
+        want = conv_reference(cut(dout), cut(x), w, bias)
+        # a channel's dbias may be a small rest of its terms, whose rounding is relative to them
+        pre = torch.nn.functional.conv1d(torch.nn.functional.pad(cut(x).double(), (kernel - 1, 0)),
+                                         w.double()[:, None], bias.double(), groups=dim)
+        s = torch.sigmoid(pre)
+        terms = (cut(dout).double() * s * (1 + pre * (1 - s))).norm() / want["db"].norm()
+        assert rel(cut(dx), want["dx"]) <= (BF16_TOL if dtype == torch.bfloat16 else TOL), off
+        assert rel(dw, want["dw"]) <= TOL, off
+        assert rel(db, want["db"]) <= TOL * max(1.0, float(terms)), off
+        assert torch.equal(dx[:off], guard[:off]) and torch.equal(dx[off + n:], guard[off + n:])
