@@ -178,6 +178,8 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None,
                     for t in (u, delta, B, C, z))
             and any(t is not None and t.requires_grad for t in given)):
         from .training import _ScanBf16
+        # moved here, so that a gradient goes back to where its input is
+        given = [None if t is None else t.to(dev) for t in given]
         out, last_state = _ScanBf16.apply(*given, bool(delta_softplus), bool(reverse))
     else:
         out, last_state = _selective_scan_op(

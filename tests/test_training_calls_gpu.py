@@ -52,3 +52,36 @@ def test_conv_backward_of_tensors_that_lie_alike_off_a_boundary(batch, dim, leng
         assert rel(dw, want["dw"]) <= TOL, off
         assert rel(db, want["db"]) <= TOL * max(1.0, float(terms)), off
         assert torch.equal(dx[:off], guard[:off]) and torch.equal(dx[off + n:], guard[off + n:])
+
+
+
+# ---------------------------------------------------------------------------
+# selective scan
+def bf16_scan(seed, lead=(), device="cuda"):
+    """Arguments of a scan with bfloat16 activations; ``lead``: further leading axes of these."""
+    g = gen(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    act = lambda *s: r(*lead, *s).to(torch.bfloat16)  # noqa: E731
+    b, d, length, n = 2, 40, 50, 16
+    inp = dict(u=act(b, d, length), delta=act(b, d, length),
+               A=-torch.arange(1, n + 1, device="cuda").float().repeat(d, 1),
+               B=act(b, 1, n, length), C=act(b, 1, n, length), D=r(d), z=act(b, d, length),
+               delta_bias=r(d) - 3, initial_state=r(b, d, n))
+    return inp, r(b, d, length), r(b, d, n)
+
+
+def test_bf16_scan_differentiates_small_inputs_of_another_device():
+    inp, dout, dlast = bf16_scan(1)
+
+    def grads(where):
+        leaves = {k: (t.to(where) if t.dtype == torch.float32 else t).clone().requires_grad_()
+                  for k, t in inp.items()}
+        out, last = arm().selective_scan(**leaves, delta_softplus=True, return_last_state=True)
+        ((out * dout).sum() + (last * dlast).sum()).backward()
+        return {k: t.grad for k, t in leaves.items()}
+
+    want, got = grads("cuda"), grads("cpu")
+    for k, t in got.items():
+        assert t.dtype == inp[k].dtype
+        assert t.device.type == ("cpu" if inp[k].dtype == torch.float32 else "cuda"), k
+        assert torch.equal(t.cpu(), want[k].cpu()), k
