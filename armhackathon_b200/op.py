@@ -460,7 +460,8 @@ def causal_conv1d_silu(x, weight, bias=None):
         raise ValueError("causal_conv1d_silu takes a (batch, dim, len) CUDA tensor")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         from .training import _ConvSilu
-        return _ConvSilu.apply(x, weight, bias)
+        # moved here, so that a gradient goes back to where its input is
+        return _ConvSilu.apply(*[None if t is None else t.to(x.device) for t in (x, weight, bias)])
     return _causal_conv1d_silu(x, weight, bias)
 
 

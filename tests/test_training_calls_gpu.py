@@ -54,6 +54,19 @@ def test_conv_backward_of_tensors_that_lie_alike_off_a_boundary(batch, dim, leng
         assert torch.equal(dx[:off], guard[:off]) and torch.equal(dx[off + n:], guard[off + n:])
 
 
+def test_conv_differentiates_weights_of_another_device():
+    g = gen(8)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x, w, bias, dout = r(2, 12, 60), r(12, 1, 4), r(12), r(2, 12, 60)
+
+    def grads(where):
+        leaves = [t.clone().requires_grad_() for t in (x, w.to(where), bias.to(where))]
+        (arm().causal_conv1d_silu(*leaves) * dout).sum().backward()
+        return [t.grad for t in leaves]
+
+    for got, want, where in zip(grads("cpu"), grads("cuda"), ("cuda", "cpu", "cpu")):
+        assert got.device.type == where and torch.equal(got.cpu(), want.cpu())
+
 
 # ---------------------------------------------------------------------------
 # selective scan
