@@ -61,20 +61,8 @@ class _on_device:
             self.ctx.__exit__(*exc)
 
 
-@torch.library.custom_op("arm_scan::selective_scan", mutates_args=())
-def _selective_scan_op(
-    u: torch.Tensor,
-    delta: torch.Tensor,
-    a: torch.Tensor,
-    b: torch.Tensor,
-    c: torch.Tensor,
-    d_skip: Optional[torch.Tensor],
-    z: Optional[torch.Tensor],
-    delta_bias: Optional[torch.Tensor],
-    h0: Optional[torch.Tensor],
-    delta_softplus: bool,
-    reverse: bool,
-) -> Tuple[torch.Tensor, torch.Tensor]:
+def _selective_scan(u, delta, a, b, c, d_skip, z, delta_bias, h0, delta_softplus, reverse):
+    """(out, last_state) of contiguous fp32 tensors on one device."""
     batch, dim, length = u.shape
     state = a.shape[1]
     groups = b.shape[1] if b.dim() == 4 else 1
@@ -89,6 +77,23 @@ def _selective_scan_op(
             stream=_stream(u))
     _CALLS["n"] += 1
     return out, last_state
+
+
+@torch.library.custom_op("arm_scan::selective_scan", mutates_args=())
+def _selective_scan_op(
+    u: torch.Tensor,
+    delta: torch.Tensor,
+    a: torch.Tensor,
+    b: torch.Tensor,
+    c: torch.Tensor,
+    d_skip: Optional[torch.Tensor],
+    z: Optional[torch.Tensor],
+    delta_bias: Optional[torch.Tensor],
+    h0: Optional[torch.Tensor],
+    delta_softplus: bool,
+    reverse: bool,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _selective_scan(u, delta, a, b, c, d_skip, z, delta_bias, h0, delta_softplus, reverse)
 
 
 @_selective_scan_op.register_fake
@@ -141,6 +146,45 @@ def _selective_scan_grad(ctx, dout, dlast):
 _selective_scan_op.register_autograd(_selective_scan_grad, setup_context=_selective_scan_setup)
 
 
+# The same on bfloat16 activations that need gradients, for calls that are traced or mapped:
+# computed in fp32 as ever, but the tensors kept for the backward are the bfloat16 ones.
+@torch.library.custom_op("arm_scan::selective_scan_bf16", mutates_args=())
+def _selective_scan_bf16_op(
+    u: torch.Tensor,
+    delta: torch.Tensor,
+    a: torch.Tensor,
+    b: torch.Tensor,
+    c: torch.Tensor,
+    d_skip: Optional[torch.Tensor],
+    z: Optional[torch.Tensor],
+    delta_bias: Optional[torch.Tensor],
+    h0: Optional[torch.Tensor],
+    delta_softplus: bool,
+    reverse: bool,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _selective_scan(*[None if t is None else _prep(t, u.device) for t in
+                             (u, delta, a, b, c, d_skip, z, delta_bias, h0)],
+                           delta_softplus, reverse)
+
+
+@_selective_scan_bf16_op.register_fake
+def _(u, delta, a, b, c, d_skip, z, delta_bias, h0, delta_softplus, reverse):
+    f32 = torch.float32
+    return (torch.empty_like(u, dtype=f32),
+            u.new_empty((u.shape[0], u.shape[1], a.shape[1]), dtype=f32))
+
+
+_selective_scan_bf16_op.register_autograd(_selective_scan_grad,
+                                          setup_context=_selective_scan_setup)
+
+
+def _traced():
+    """Whether calls are recorded (compile, export, make_fx) or mapped (torch.func) instead of
+    run: only custom ops pass through these."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or torch._C._functorch.peek_interpreter_stack() is not None)
+
+
 def _bc4(t, batch, state, length):
     return t.reshape(batch, 1, state, length) if t.dim() == 3 else t
 
@@ -173,14 +217,23 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None,
     B = B.reshape(lay.bc_shape)
     C = C.reshape(lay.bc_shape)
     given = (u, delta, A, B, C, D, z, delta_bias, initial_state)
+    traced = _traced()
     if (dev.type == "cuda" and torch.is_grad_enabled()
             and all(t is None or (t.dtype == torch.bfloat16 and t.device == dev)
                     for t in (u, delta, B, C, z))
-            and any(t is not None and t.requires_grad for t in given)):
-        from .training import _ScanBf16
+            and any(t is not None and t.requires_grad for t in given)
+            # jit.trace compares its graph with one recorded without gradients
+            and (traced or not torch.jit.is_tracing())):
         # moved here, so that a gradient goes back to where its input is
-        given = [None if t is None else t.to(dev) for t in given]
-        out, last_state = _ScanBf16.apply(*given, bool(delta_softplus), bool(reverse))
+        given = [None if t is None else t.to(dev).contiguous() for t in given]
+        if traced:
+            run = _selective_scan_bf16_op
+        else:
+            # the same without the two ops' dispatch, which is most of a short call: forward and
+            # backward of 2 x 128 rows of 77 steps 280 us, through the ops 375
+            from .training import _ScanBf16
+            run = _ScanBf16.apply
+        out, last_state = run(*given, bool(delta_softplus), bool(reverse))
     else:
         out, last_state = _selective_scan_op(
             *[None if t is None else _prep(t, dev) for t in given], bool(delta_softplus),

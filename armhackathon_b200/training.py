@@ -28,7 +28,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _ffi
 from .layout import m1_layout
-from .op import _CALLS, _causal_conv1d_silu, _prep, _ptr, _selective_scan_op
+from .op import _CALLS, _causal_conv1d_silu, _prep, _ptr, _selective_scan
 
 _DTYPES = {torch.float32: _ffi.DTYPE_F32, torch.bfloat16: _ffi.DTYPE_BF16}
 _NO_GUARD = contextlib.nullcontext()
@@ -161,27 +161,26 @@ def selective_scan_backward(dout, u, delta, A, B, C, D=None, z=None, delta_bias=
 
 
 class _ScanBf16(torch.autograd.Function):
-    """``selective_scan`` on bfloat16 activations with gradients: the forward
-    runs in fp32 as ever, the bfloat16 tensors are what is kept."""
+    """``selective_scan`` on contiguous bfloat16 activations with gradients: the
+    forward runs in fp32 as ever, the bfloat16 tensors are what is kept."""
 
     @staticmethod
     def forward(ctx, u, delta, A, B, C, D, z, delta_bias, h0, delta_softplus, reverse):
-        acts = [None if t is None else t.contiguous() for t in (u, delta, B, C, z)]
-        ctx.save_for_backward(*acts, A, D, delta_bias, h0)
+        given = (u, delta, A, B, C, D, z, delta_bias, h0)
+        ctx.save_for_backward(*given)
         ctx.flags = (delta_softplus, reverse)
         ctx.set_materialize_grads(False)
-        opt = lambda t: None if t is None else _prep(t, u.device)  # noqa: E731
-        return _selective_scan_op(*[opt(t) for t in (u, delta, A, B, C, D, z, delta_bias, h0)],
-                                  delta_softplus, reverse)
+        return _selective_scan(*[None if t is None else _prep(t, u.device) for t in given],
+                               delta_softplus, reverse)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dlast):
-        u, delta, B, C, z, A, D, delta_bias, h0 = ctx.saved_tensors
+        given = ctx.saved_tensors
         if dout is None:  # only the last state is used
-            dout = torch.zeros_like(u)
-        return (*selective_scan_backward(dout, u, delta, A, B, C, D, z, delta_bias, ctx.flags[0], h0,
-                                         dlast, ctx.flags[1]), None, None)
+            dout = torch.zeros_like(given[0])
+        return (*selective_scan_backward(dout, *given[:8], ctx.flags[0], given[8], dlast,
+                                         ctx.flags[1]), None, None)
 
 
 # ---------------------------------------------------------------------------

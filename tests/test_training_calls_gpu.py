@@ -70,7 +70,7 @@ def test_conv_differentiates_weights_of_another_device():
 
 # ---------------------------------------------------------------------------
 # selective scan
-def bf16_scan(seed, lead=(), device="cuda"):
+def bf16_scan(seed, lead=()):
     """Arguments of a scan with bfloat16 activations; ``lead``: further leading axes of these."""
     g = gen(seed)
     r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
@@ -98,3 +98,50 @@ def test_bf16_scan_differentiates_small_inputs_of_another_device():
         assert t.dtype == inp[k].dtype
         assert t.device.type == ("cpu" if inp[k].dtype == torch.float32 else "cuda"), k
         assert torch.equal(t.cpu(), want[k].cpu()), k
+
+
+def test_bf16_scan_traces_in_one_graph():
+    inp, dout, dlast = bf16_scan(2)
+
+    def call(inp):
+        return arm().selective_scan(**inp, delta_softplus=True, return_last_state=True)
+
+    def grads(f):
+        leaves = {k: t.clone().requires_grad_() for k, t in inp.items()}
+        out, last = f(leaves)
+        ((out * dout).sum() + (last * dlast).sum()).backward()
+        return [out, last, *[t.grad for t in leaves.values()]]
+
+    torch._dynamo.reset()
+    want = grads(call)
+    got = grads(torch.compile(call, fullgraph=True, backend="aot_eager"))
+    assert all(p.dtype == q.dtype and torch.equal(p, q) for p, q in zip(got, want))
+    # one parameter of an evaluated model that requires grad is enough
+    some = {**inp, "A": inp["A"].clone().requires_grad_()}
+    out, _ = torch.compile(call, fullgraph=True, backend="aot_eager")(some)
+    assert torch.equal(out, want[0])
+
+
+def test_bf16_scan_maps_over_an_axis():
+    inp, _, _ = bf16_scan(3, lead=(3,))
+    inp["A"].requires_grad_()
+    acts = [inp[k] for k in ("u", "delta", "B", "C", "z")]
+
+    def call(u, delta, B, C, z):
+        return arm().selective_scan(u, delta, inp["A"], B, C, D=inp["D"], z=z,
+                                    delta_bias=inp["delta_bias"], delta_softplus=True)
+
+    got = torch.func.vmap(call)(*acts)
+    want = torch.stack([call(*[t[i] for t in acts]) for i in range(3)])
+    assert torch.equal(got, want)
+
+
+def test_bf16_scan_op_checks():
+    inp, _, _ = bf16_scan(4)
+    args = [inp[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "initial_state")]
+    args = [t.clone().requires_grad_() for t in args]
+    checks = ("test_schema", "test_autograd_registration", "test_faketensor",
+              "test_aot_dispatch_dynamic")
+    for flags in ((True, False), (True, True)):
+        torch.library.opcheck(torch.ops.arm_scan.selective_scan_bf16, (*args, *flags),
+                              test_utils=checks)
