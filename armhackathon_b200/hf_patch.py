@@ -115,7 +115,17 @@ def _conv_silu(mixer, hidden):
     return mixer.act(mixer.conv1d(hidden)[..., :hidden.shape[-1]])
 
 
-def _prefill(mixer, x, cache_params, cache_position, attention_mask, api):
+def _scan_dtype(mixer, hidden, u, train):
+    """Type in which x_proj and the scan read the conv's fp32 output ``u``: as it is where
+    x_proj takes it; the activations' where x_proj is a product in that type, and in training
+    under autocast, so that the scan keeps 16-bit tensors for its gradients."""
+    if torch.is_autocast_enabled(hidden.device.type):
+        return hidden.dtype if train else u.dtype
+    weight = getattr(mixer.x_proj, "weight", None)
+    return hidden.dtype if weight is not None and weight.dtype == hidden.dtype else u.dtype
+
+
+def _prefill(mixer, x, cache_params, cache_position, attention_mask, api, train=False):
     seq_len = x.shape[1]
     out_dtype = x.dtype
     hidden, gate = mixer.in_proj(x).transpose(1, 2).chunk(2, dim=1)
@@ -128,7 +138,8 @@ def _prefill(mixer, x, cache_params, cache_position, attention_mask, api):
             cache_params.update_conv_state(mixer.layer_idx, window, cache_position)
         else:
             cache_params.update_conv_state(window, mixer.layer_idx)
-    u = _conv_silu(mixer, hidden.contiguous()).to(hidden.dtype)
+    u = _conv_silu(mixer, hidden.contiguous())
+    u = u.to(_scan_dtype(mixer, hidden, u, train))
     if attention_mask is not None:
         u = u * attention_mask.unsqueeze(1)
     proj = mixer.x_proj(u.transpose(1, 2))
@@ -190,7 +201,7 @@ def _install_mixer(modeling_mamba):
             else:
                 counters.train_calls += 1
             return _prefill(self, input_states, cache_params, cache_position,
-                            kw.get("attention_mask"), api)
+                            kw.get("attention_mask"), api, route == "train")
         if route == "decode":
             counters.decode_calls += 1
             return _decode(self, input_states, cache_params, kw.get("attention_mask"))

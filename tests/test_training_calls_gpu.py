@@ -145,3 +145,93 @@ def test_bf16_scan_op_checks():
     for flags in ((True, False), (True, True)):
         torch.library.opcheck(torch.ops.arm_scan.selective_scan_bf16, (*args, *flags),
                               test_utils=checks)
+
+
+# ---------------------------------------------------------------------------
+# the patch in 16 bits
+def tiny_mamba(dtype=torch.float32):
+    from transformers import MambaConfig, MambaForCausalLM
+    cfg = MambaConfig(vocab_size=500, hidden_size=64, state_size=16, num_hidden_layers=2, expand=2,
+                      conv_kernel=4, time_step_rank=8, use_cache=False)
+    torch.manual_seed(0)
+    return MambaForCausalLM(cfg).cuda().to(dtype)
+
+
+@pytest.fixture
+def seen(monkeypatch):
+    """The conv's outputs and what the scan is given, call by call."""
+    from armhackathon_b200 import hf_patch
+    conv, scan, got = hf_patch.causal_conv1d_silu, hf_patch.selective_scan, []
+
+    def conv1d(*a):
+        got.append([conv(*a)])
+        return got[-1][0]
+
+    def selective_scan(u, *a, **kw):
+        got[-1].append(u)
+        return scan(u, *a, **kw)
+
+    monkeypatch.setattr(hf_patch, "causal_conv1d_silu", conv1d)
+    monkeypatch.setattr(hf_patch, "selective_scan", selective_scan)
+    return got
+
+
+def patched(call, training=False):
+    assert arm().patch(training=training)
+    try:
+        return call()
+    finally:
+        assert arm().unpatch()
+
+
+def test_patched_inference_under_autocast_scans_the_conv_in_32_bits(seen):
+    model = tiny_mamba().eval()
+    ids = torch.randint(0, 500, (2, 33), device="cuda")
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        logits = patched(lambda: model(ids).logits)
+    assert len(seen) == 2 and torch.isfinite(logits).all()
+    for conv, u in seen:
+        assert u.dtype == torch.float32 and torch.equal(u, conv)
+
+
+@pytest.mark.parametrize("own_x_proj", [False, True])
+def test_patched_inference_of_a_bf16_model(seen, own_x_proj):
+    # 16-bit weights throughout, or with an x_proj that is kept in fp32
+    model = tiny_mamba(torch.bfloat16).eval()
+    ids = torch.randint(0, 500, (2, 33), device="cuda")
+    with torch.no_grad():
+        if own_x_proj:
+            from torch import nn
+
+            class Wide(nn.Linear):
+                def forward(self, x):
+                    return super().forward(x).to(torch.bfloat16)
+
+            for block in model.backbone.layers:
+                p = block.mixer.x_proj
+                wide = Wide(p.in_features, p.out_features, bias=False).cuda()
+                wide.weight.copy_(p.weight.float())
+                block.mixer.x_proj = wide
+        got = patched(lambda: model(ids).logits)
+        assert len(seen) == 2 and torch.isfinite(got).all()
+        for conv, u in seen:
+            assert u.dtype == (torch.float32 if own_x_proj else torch.bfloat16)
+            assert torch.equal(u, conv.to(u.dtype))
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+def test_patched_training_in_16_bits(seen, autocast):
+    model = tiny_mamba(torch.float32 if autocast else torch.bfloat16).train()
+    ids = torch.randint(0, 500, (2, 33), device="cuda")
+
+    def step():
+        model.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            loss = model(ids, labels=ids).loss
+        loss.backward()
+        return {n: p.grad for n, p in model.named_parameters()}
+
+    grads = patched(step, training=True)
+    assert len(seen) == 2 and all(u.dtype == torch.bfloat16 for _, u in seen)
+    for n, p in model.named_parameters():
+        assert grads[n].dtype == p.dtype and torch.isfinite(grads[n]).all(), n
