@@ -273,6 +273,11 @@ def _norm_args(what, x, weight, residual, residual_dtype):
     return dev, head, res_out, (xr, rr, w)
 
 
+def _needs_grad(x, weight, residual):
+    return torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                        (residual is not None and residual.requires_grad))
+
+
 def _add_rms_norm(x, weight, residual, eps, residual_dtype, want_rstd):
     dev, head, res_out, held = _norm_args("add_rms_norm", x, weight, residual, residual_dtype)
     y = _new(x, x.dtype)
@@ -314,8 +319,7 @@ def add_rms_norm(x, weight, residual=None, eps=1e-5, residual_dtype=None, return
     x's type (``residual_dtype`` chooses it when there is no residual).  weight
     (dim,).  The norm is taken from the fp32 sum before residual_out is
     rounded.  rstd (...) is what ``add_rms_norm_backward`` takes.  Differentiable."""
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
-                                    (residual is not None and residual.requires_grad)):
+    if _needs_grad(x, weight, residual):
         y, res_out, rstd = _AddRmsNorm.apply(x, weight, residual, float(eps), residual_dtype)
     else:
         y, res_out, rstd = _add_rms_norm(x, weight, residual, float(eps), residual_dtype,
@@ -323,19 +327,37 @@ def add_rms_norm(x, weight, residual=None, eps=1e-5, residual_dtype=None, return
     return (y, res_out, rstd) if return_rstd else (y, res_out)
 
 
-def add_rms_norm_fp8(x, weight, residual=None, eps=1e-5, residual_dtype=None):
-    """``add_rms_norm`` with the output in 8 bits: returns (y8, scale,
-    residual_out), y8 float8_e4m3fn (..., dim) and scale float32 (...) with
-    y = y8 * scale, scale = max|y| / 448 per row, at least 2^-126 (1 for a row of
-    zeros).  The row-scaled operand of an 8-bit projection; inference only."""
+def _add_rms_norm_fp8(x, weight, residual, eps, residual_dtype):
     dev, head, res_out, held = _norm_args("add_rms_norm_fp8", x, weight, residual, residual_dtype)
     y8 = _new(x, torch.float8_e4m3fn)
     scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     with _guard(dev):
-        _ffi.add_rms_norm_fp8_raw(*head, float(eps), y8.data_ptr(), scale.data_ptr(),
-                                  res_out.data_ptr(), _stream(dev))
+        _ffi.add_rms_norm_fp8_raw(*head, eps, y8.data_ptr(), scale.data_ptr(), res_out.data_ptr(),
+                                  _stream(dev))
     del held
     return y8, scale, res_out
+
+
+class _AddRmsNormFp8(torch.autograd.Function):
+    """No gradient exists: a backward that reaches any output raises."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _add_rms_norm_fp8(*args)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("add_rms_norm_fp8 has no gradient: use add_rms_norm where one is needed")
+
+
+def add_rms_norm_fp8(x, weight, residual=None, eps=1e-5, residual_dtype=None):
+    """``add_rms_norm`` with the output in 8 bits: returns (y8, scale,
+    residual_out), y8 float8_e4m3fn (..., dim) and scale float32 (...) with
+    y = y8 * scale, scale = max|y| / 448 per row, at least 2^-126 (1 for a row of
+    zeros).  The row-scaled operand of an 8-bit projection; inference only: a
+    backward through any output raises."""
+    run = _AddRmsNormFp8.apply if _needs_grad(x, weight, residual) else _add_rms_norm_fp8
+    return run(x, weight, residual, float(eps), residual_dtype)
 
 
 def add_rms_norm_backward(dy, residual_out, weight, rstd, dresidual_out=None):

@@ -235,3 +235,23 @@ def test_patched_training_in_16_bits(seen, autocast):
     assert len(seen) == 2 and all(u.dtype == torch.bfloat16 for _, u in seen)
     for n, p in model.named_parameters():
         assert grads[n].dtype == p.dtype and torch.isfinite(grads[n]).all(), n
+
+
+# ---------------------------------------------------------------------------
+# RMS norm
+def test_norm_fp8_refuses_gradients():
+    x = torch.randn(6, 64, device="cuda", generator=gen(5))
+    res, w = torch.randn(6, 64, device="cuda", generator=gen(6)), torch.ones(64, device="cuda")
+    want = arm().add_rms_norm_fp8(x, w, residual=res)
+    for leaf in (x, w, res):
+        leaf.requires_grad_()
+        got = arm().add_rms_norm_fp8(x, w, residual=res)  # the call itself runs as ever
+        for p, q in zip(got, want):
+            assert p.dtype == q.dtype and torch.equal(p.detach().float(), q.float())
+        for t in got:  # and no gradient is dropped on the way back
+            with pytest.raises(RuntimeError, match="add_rms_norm_fp8"):
+                t.float().sum().backward()
+        with torch.no_grad():
+            assert not any(t.requires_grad for t in arm().add_rms_norm_fp8(x, w, residual=res))
+        leaf.requires_grad_(False)
+    assert not any(t.requires_grad for t in want)
