@@ -421,7 +421,8 @@ def _clip(what, grads, max_norm, eps, scale):
     if len(devices) > 1 or dev.type != "cuda":
         raise ValueError(f"{what} runs on CUDA tensors of one device, got "
                          f"{sorted({str(g.device) for g in grads})}")
-    other = set(dtypes) - _DTYPES.keys()
+    kinds = set(dtypes)
+    other = kinds - _DTYPES.keys()
     if other:
         raise ValueError(f"{what} takes float32 and bfloat16 gradients, got {other.pop()}")
     if not all(map(torch.Tensor.is_contiguous, grads)):
@@ -429,14 +430,18 @@ def _clip(what, grads, max_norm, eps, scale):
             if not (g.is_contiguous() or _dense(g)):
                 raise ValueError(f"{what}: a gradient of shape {tuple(g.shape)} and strides "
                                  f"{g.stride()} does not fill its memory")
+    # most lists hold one type: looking each up took 2 us of 32 tensors' call
+    codes = (array("i", (_DTYPES[dtypes[0]],)) * len(grads) if len(kinds) == 1
+             else array("i", map(_DTYPES.__getitem__, dtypes)))
     norm = torch.empty((), dtype=torch.float32, device=dev)
     with _guard(dev):
         nbytes = _ffi.clip_grads_workspace_bytes()
         ws = _workspace(nbytes, norm)
         _ffi.clip_grads_raw(array("Q", map(torch.Tensor.data_ptr, grads)),
-                            array("Q", map(torch.Tensor.numel, grads)),
-                            array("i", map(_DTYPES.__getitem__, dtypes)), max_norm, eps, scale,
+                            array("Q", map(torch.Tensor.numel, grads)), codes, max_norm, eps, scale,
                             ws.data_ptr(), nbytes, norm.data_ptr(), _stream(dev))
+    if scale:  # autograd notices tensors that it kept, as with torch's in-place operations
+        torch.autograd.graph.increment_version(grads)
     return norm
 
 

@@ -255,3 +255,20 @@ def test_norm_fp8_refuses_gradients():
             assert not any(t.requires_grad for t in arm().add_rms_norm_fp8(x, w, residual=res))
         leaf.requires_grad_(False)
     assert not any(t.requires_grad for t in want)
+
+
+# ---------------------------------------------------------------------------
+# clipping
+def test_clip_is_noticed_by_autograd():
+    p = torch.randn(50, device="cuda", generator=gen(7)).requires_grad_()
+    g, = torch.autograd.grad((p ** 3).sum(), p, create_graph=True)
+    penalty = (g * g).sum()  # keeps g for its own gradient
+    before = g._version
+    arm().grad_norm([g.detach()])
+    assert g._version == before
+    arm().clip_grads_([g.detach(), torch.ones(3, device="cuda")], 0.1)
+    assert g._version > before
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        penalty.backward()
+    with torch.inference_mode():
+        arm().clip_grads_([torch.ones(3, device="cuda")], 0.1)
