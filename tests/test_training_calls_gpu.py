@@ -8,7 +8,8 @@ same kernels on the same values are bitwise.
 import pytest
 import torch
 
-from test_training_gpu import BF16_TOL, TOL, conv_reference, gen, rel
+from test_training_gpu import (BF16_TOL, EPS, NORM_TYPES, TOL, check, conv_reference, gen,
+                               norm_inputs, rel)
 
 pytestmark = pytest.mark.gpu
 
@@ -52,6 +53,21 @@ def test_conv_backward_of_tensors_that_lie_alike_off_a_boundary(batch, dim, leng
         assert rel(dw, want["dw"]) <= TOL, off
         assert rel(db, want["db"]) <= TOL * max(1.0, float(terms)), off
         assert torch.equal(dx[:off], guard[:off]) and torch.equal(dx[off + n:], guard[off + n:])
+
+
+@pytest.mark.parametrize("length", [64, 77])
+def test_conv_autograd_in_16_bits(length):
+    g = gen(length)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x, w, bias, dout = r(2, 30, length).to(torch.bfloat16), r(30, 4), r(30), r(2, 30, length)
+    want = conv_reference(dout, x, w, bias)
+    leaves = [t.clone().requires_grad_() for t in (x, w, bias)]
+    out = arm().causal_conv1d_silu(*leaves)
+    assert out.dtype == torch.float32
+    (out * dout).sum().backward()
+    got = [t.grad for t in leaves]
+    assert got[0].dtype == torch.bfloat16
+    check(dict(zip(("dx", "dw", "db"), got)), want, TOL)
 
 
 def test_conv_differentiates_weights_of_another_device():
@@ -272,3 +288,74 @@ def test_clip_is_noticed_by_autograd():
         penalty.backward()
     with torch.inference_mode():
         arm().clip_grads_([torch.ones(3, device="cuda")], 0.1)
+
+
+# ---------------------------------------------------------------------------
+# several turns of the persistent loops
+@pytest.mark.parametrize("types", NORM_TYPES)
+@pytest.mark.parametrize("rows,dim", [(4001, 40), (4001, 768), (4001, 33), (1501, 1030), (1501, 2560),
+                                      (701, 5000), (701, 4099)])
+def test_norm_backward_of_many_rows(rows, dim, types):
+    # each warp or CTA takes several rows and the last turn is not full: rows loaded ahead, the
+    # alternating buffer of the sums, dw in registers
+    x, res, w = norm_inputs(rows, dim, types, seed=dim)
+    dy, extra, _ = norm_inputs(rows, dim, types, seed=dim + 1)
+    stored = (res.double().square().mean(-1) + EPS).rsqrt().float()
+    for dres in (extra, None):
+        rl, wl = res.double().requires_grad_(), w.double().requires_grad_()
+        y = rl * (rl.square().mean(-1, keepdim=True) + EPS).rsqrt() * wl
+        total = (y * dy.double()).sum() + (0 if dres is None else (rl * dres.double()).sum())
+        wantr, wantw = torch.autograd.grad(total, [rl, wl])
+        dx, dr, dw = arm().add_rms_norm_backward(dy, res, w, stored, dresidual_out=dres)
+        # a difference: its rounding is relative to its parts
+        parts = float((dy.double() * w.double() * stored.double()[:, None]).norm() / wantr.norm())
+        check({"dx": dx, "dr": dr, "dw": dw}, {"dx": wantr, "dr": wantr, "dw": wantw},
+              TOL * max(1.0, parts))
+        # and row by row, so that one stale row shows
+        off = (dr.double() - wantr).norm(dim=-1) / wantr.norm(dim=-1)
+        assert float(off.max()) <= (BF16_TOL if dr.dtype == torch.bfloat16 else 4 * TOL)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clip_of_more_chunks_than_ctas(dtype):
+    sizes = [9_000_001, 5, 7_654_321, 16384 * 200 + 3]
+    flat = torch.randn(sum(sizes) + 1, device="cuda", generator=gen(9)).to(dtype)
+    grads = list(torch.split(flat[1:], sizes))
+    first, before = flat[0].clone(), flat[1:].double()
+    norm = arm().clip_grads_(grads, 2.0)
+    want = before.norm()
+    assert rel(norm, want) <= TOL
+    # one factor (3 roundings) and a product, each value on its own
+    lim = (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -22) * before.abs() * float(2 / want)
+    lim = lim + (1e-38 if dtype == torch.bfloat16 else 1e-44)
+    assert ((flat[1:].double() - before * float(2 / (want + 1e-6))).abs() <= lim).all()
+    assert torch.equal(flat[0], first)
+
+
+@pytest.mark.parametrize("tensors", [3, 700])
+def test_clip_captured_in_a_graph(tensors):
+    a = arm()
+    values = [torch.randn(40 + i, device="cuda", generator=gen(i)) for i in range(tensors)]
+    grads = [torch.empty_like(v) for v in values]
+
+    def fill(scale):
+        for p, v in zip(grads, values):
+            p.copy_(v * scale)
+
+    fill(1.0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a.clip_grads_(grads, 0.5)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = a.clip_grads_(grads, 0.5)
+    for scale in (1.0, 3.0, 1e-5):
+        fill(scale)
+        want_norm = a.clip_grads_(grads, 0.5)
+        want = [p.clone() for p in grads]
+        fill(scale)
+        graph.replay()
+        assert torch.equal(norm, want_norm)
+        assert all(torch.equal(p, q) for p, q in zip(grads, want))
