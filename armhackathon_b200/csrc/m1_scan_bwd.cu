@@ -34,8 +34,9 @@
 //
 // Measured at 8 x 1536 rows of 2048 steps, 16 states, fp32: 760 us (sweep 222,
 // carries 10, main 530, sums 20 when timed apart).  Floors: 709 MB at 6.55 TB/s 108
-// us, 9.9 GFLOP at the fp32 pipes' 72 TFLOP/s 137 us, two exponentials per (row,
-// step, state) at 16 a cycle and SM 179 us.  What binds it is latency: the main
+// us, 9.9 GFLOP at the fp32 pipes' 72 TFLOP/s 137 us.  The passes' own decays, two
+// per (row, step, state) and, in rows cut into segments, one per block of four
+// steps, take 201 us at 16 exponentials a cycle and SM.  What binds it is latency: the main
 // kernel issues on 53% of cycles with 3 warps a scheduler (168 registers: a and
 // a h_{t-1} of eight pairs over four steps are 64 of them), its shared-memory
 // path is 61% busy, FP32 pipes 42%, MUFU 31%, HBM 25%.  Of its time the
@@ -58,7 +59,7 @@ constexpr int kTile = 16;    // steps staged at a time
 constexpr int kTileBlocks = kTile / kT;
 constexpr int kWarps = 4;
 constexpr int kRowsW = 16;   // rows of a warp
-constexpr int kRowsC = kWarps * kRowsW;
+constexpr int kRowsC = kWarps * kRowsW;    // rows of a CTA: a group's channels are padded to it
 constexpr int kThreads = kWarps * 32;
 constexpr int kStates = 16;
 constexpr int kRowPitch = kTile + 4;       // floats between rows of a staged tensor
@@ -100,15 +101,16 @@ Plan make_plan(const M1BwdParams& p) {
     q.tiles = (p.len + kTile - 1) / kTile;
     // Segments: of at most 128 steps, since the roundings of the decays add up along
     // a recurrence, and a carry between segments takes one decay of summed dt instead
-    // (error of dA, 8 x 1536 rows of 2048 steps: 1.07e-6 in 10 segments, 9.4e-7 in 16;
-    // with a scan by doubling spans in fp32 7.0e-7.  1 x 1536 rows of 32768: 1.25e-6 in
-    // 128, 1.04e-6 in 256; 1.09e-6).  Among the numbers that give the SMs 1, 2, .. 36
+    // (error of dA, 8 x 1536 rows of 2048 steps: 1.07e-6 in 10 segments, 9.3e-7 in 16;
+    // with a scan by doubling spans in fp32 7.3e-7.  1 x 1536 rows of 32768: 1.20e-6 in
+    // 128, 9.9e-7 in 256; 1.02e-6).  Among the numbers that give the SMs 1, 2, .. 36
     // CTAs each, the one with the least estimated time: a tile takes 7, 9 or 12 units
     // with 1, 2 or 3 CTAs on its SM; full waves run at 3, the rest at what is left; a
     // CTA's start-up and the carries count as one and a half tiles; CTAs that all
     // start together stay in step and get in each other's way (a tenth, over the
     // number of waves).  Measured, the same rows: 16 segments 760 us, 13: 746, 32:
-    // 794; 256 segments 1453 us, 128: 1421, 410: 1504.
+    // 794; 256 segments 1453 us, 128: 1421, 410: 1504.  (The units were fitted to 16
+    // states in fp32 and serve every state count and type.)
     q.seg_tiles = q.tiles;
     if (const int forced = kernel_override(kKnobM1Segments)) {
         q.seg_tiles = (q.tiles + forced - 1) / forced;
@@ -373,9 +375,9 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // A of a row slot's four states.  A decay is 2^(A (dt log2(e))): A itself stays
-// exact, since an error of the factor common to all of a row's steps would add up
-// over them (with A log2(e) rounded once, dA of 1 x 1536 rows of 32768 steps was 1.26e-6
-// off instead of 1.19e-6 in 128 segments).
+// exact, so that no rounding of the factor common to all of a row's steps adds up
+// over them (at A = -1 .. -16 none is seen to: dA of 1 x 1536 rows of 32768 steps in 128
+// segments is 1.2e-6 off with A log2(e) rounded, too).
 __device__ __forceinline__ void load_a(const M1BwdParams& p, const Lane& l, int64_t n0, int k, float2* A) {
     float v[4];
 #pragma unroll

@@ -18,7 +18,8 @@ There is no CPU implementation: without a GPU the call raises.
 
 ``selective_scan`` and ``causal_conv1d_silu`` differentiate on CUDA tensors
 (training.py holds the gradients); the other ops are inference only, as in the
-reference.
+reference.  ``arm_scan::selective_scan_bf16`` and ``selective_scan_backward``
+are the ops of traced calls with bfloat16 activations and of gradients.
 """
 
 from typing import List, Optional, Tuple

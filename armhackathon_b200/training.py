@@ -200,7 +200,9 @@ class _ConvSilu(torch.autograd.Function):
 def causal_conv1d_silu_backward(dout, x, weight, bias=None):
     """Gradients (dx, dweight, dbias) of ``causal_conv1d_silu``; dbias is None
     without a bias.  dout and x both bfloat16 are read (and dx written) in 16
-    bits, otherwise in float32; CUDA tensors only."""
+    bits, otherwise in float32; CUDA tensors only.  Through autograd dout is
+    float32, as the forward's output is: a bfloat16 x is then converted, and dx
+    back."""
     if x.dim() != 3:
         raise ValueError("causal_conv1d_silu_backward takes a (batch, dim, len) CUDA tensor")
     dev = _need_cuda("causal_conv1d_silu_backward", x, dout, weight, bias)
@@ -354,8 +356,10 @@ def add_rms_norm_fp8(x, weight, residual=None, eps=1e-5, residual_dtype=None):
     """``add_rms_norm`` with the output in 8 bits: returns (y8, scale,
     residual_out), y8 float8_e4m3fn (..., dim) and scale float32 (...) with
     y = y8 * scale, scale = max|y| / 448 per row, at least 2^-126 (1 for a row of
-    zeros).  The row-scaled operand of an 8-bit projection; inference only: a
-    backward through any output raises."""
+    zeros).  y8 is rounded from y times 1 / scale in fp32: within 1e-7 of the
+    middle between two 8-bit values either may be written.  The row-scaled
+    operand of an 8-bit projection; inference only: a backward through any
+    output raises."""
     run = _AddRmsNormFp8.apply if _needs_grad(x, weight, residual) else _add_rms_norm_fp8
     return run(x, weight, residual, float(eps), residual_dtype)
 
@@ -456,7 +460,8 @@ def clip_grads_(grads, max_norm, eps=1e-6):
     """Scale every gradient in place by min(1, max_norm / (norm + eps)), norm
     being ``grad_norm(grads)`` before the call, which is returned.  The rule of
     ``torch.nn.utils.clip_grad_norm_`` on the gradients themselves: a factor of
-    1 leaves every bit as it was, a NaN norm makes every gradient NaN."""
+    1 leaves every bit as it was, a NaN norm makes every gradient NaN.  Autograd
+    counts it as an in-place change."""
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     return _clip("clip_grads_", grads, max_norm, eps, True)

@@ -473,7 +473,9 @@ int arm_scan_mamba3_mixer_prologue_f32_async(const ArmMamba3MixerDims* dims, con
  * `dout_dtype` (ARM_SCAN_DTYPE_F32 or _BF16; with F32 activations dout is F32
  * too); everything else is fp32.  Nothing of the forward pass is needed but
  * its inputs.  Null: d_skip with dd, z with dz, delta_bias with ddelta_bias
- * (both or neither: code 1), h0, dlast, dh0. */
+ * (both or neither: code 1), h0, dlast, dh0.  The channels of a group are
+ * padded to 64, in work and in scratch: about 21 bytes per (row, step) at 64
+ * channels a group or more, 82 at 16, 1318 at one. */
 size_t arm_scan_selective_scan_backward_workspace_bytes(const ArmScanDims* dims);
 int arm_scan_selective_scan_backward_async(
     const ArmScanDims* dims, int dtype, int dout_dtype, const void* dout, const void* u,
@@ -500,7 +502,8 @@ int arm_scan_causal_conv1d_silu_backward_async(size_t batch, size_t dim, size_t 
  * or (BF16, BF16): res_out has the residual's, y that of x.  residual null: r
  * = x.  rstd (rows), the reciprocal root, is nullable.  The _fp8 form writes
  * y as e4m3 bytes with scale (rows) = max|y| / 448, at least 2^-126 (1 for a
- * row of zeros): y = scale * e4m3, rounded to nearest even. */
+ * row of zeros): y = scale * e4m3, y times 1 / scale in fp32 rounded to nearest
+ * even (within 1e-7 of the middle between two e4m3 values either may result). */
 int arm_scan_add_rms_norm_async(size_t rows, size_t dim, int x_dtype, int res_dtype, int weight_dtype,
                                 const void* x, size_t x_stride, const void* residual,
                                 size_t res_stride, const void* weight, float eps, void* y,
