@@ -179,11 +179,16 @@ _selective_scan_bf16_op.register_autograd(_selective_scan_grad,
                                           setup_context=_selective_scan_setup)
 
 
-def _traced():
-    """Whether calls are recorded (compile, export, make_fx) or mapped (torch.func) instead of
-    run: only custom ops pass through these."""
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _traced(tensors):
+    """Whether a call is recorded (compile, export, make_fx), mapped (torch.func) or made on
+    tensors without memory (fake ones, other subclasses) instead of run: only custom ops pass
+    through these."""
     return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or torch._C._functorch.peek_interpreter_stack() is not None)
+            or torch._C._functorch.peek_interpreter_stack() is not None
+            or any(t is not None and type(t) not in _PLAIN for t in tensors))
 
 
 def _bc4(t, batch, state, length):
@@ -218,27 +223,25 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None,
     B = B.reshape(lay.bc_shape)
     C = C.reshape(lay.bc_shape)
     given = (u, delta, A, B, C, D, z, delta_bias, initial_state)
-    traced = _traced()
+    run, keep16 = _selective_scan_op, False
     if (dev.type == "cuda" and torch.is_grad_enabled()
-            and all(t is None or (t.dtype == torch.bfloat16 and t.device == dev)
-                    for t in (u, delta, B, C, z))
-            and any(t is not None and t.requires_grad for t in given)
-            # jit.trace compares its graph with one recorded without gradients
-            and (traced or not torch.jit.is_tracing())):
-        # moved here, so that a gradient goes back to where its input is
-        given = [None if t is None else t.to(dev).contiguous() for t in given]
-        if traced:
-            run = _selective_scan_bf16_op
+            and any(t is not None and t.requires_grad for t in given)):
+        keep16 = all(t is None or (t.dtype == torch.bfloat16 and t.device == dev)
+                     for t in (u, delta, B, C, z))
+        if _traced(given):
+            run = _selective_scan_bf16_op if keep16 else _selective_scan_op
+        elif torch.jit.is_tracing():
+            keep16 = False  # jit.trace compares its graph with one recorded without gradients
         else:
-            # the same without the two ops' dispatch, which is most of a short call: forward and
-            # backward of 2 x 128 rows of 77 steps 280 us, through the ops 375
-            from .training import _ScanBf16
-            run = _ScanBf16.apply
-        out, last_state = run(*given, bool(delta_softplus), bool(reverse))
-    else:
-        out, last_state = _selective_scan_op(
-            *[None if t is None else _prep(t, dev) for t in given], bool(delta_softplus),
-            bool(reverse))
+            # the same without the ops' dispatch, which is most of a short call: forward and
+            # backward of 2 x 128 rows of 77 steps 229 us in fp32 and 258 in bf16, through the
+            # ops 310 and 375
+            from .training import _Scan
+            run = _Scan.apply
+    # moved and cast here, so that a gradient goes back to where its input is
+    given = [None if t is None else t.to(dev).contiguous() if keep16 else _prep(t, dev)
+             for t in given]
+    out, last_state = run(*given, bool(delta_softplus), bool(reverse))
     return (out, last_state) if return_last_state else out
 
 

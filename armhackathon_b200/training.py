@@ -160,9 +160,9 @@ def selective_scan_backward(dout, u, delta, A, B, C, D=None, z=None, delta_bias=
                                 for g, i, t in zip(grads, ins, given)])
 
 
-class _ScanBf16(torch.autograd.Function):
-    """``selective_scan`` on contiguous bfloat16 activations with gradients: the
-    forward runs in fp32 as ever, the bfloat16 tensors are what is kept."""
+class _Scan(torch.autograd.Function):
+    """``selective_scan`` on contiguous tensors with gradients.  The forward runs
+    in fp32; what is kept are its inputs as they are (bfloat16 activations)."""
 
     @staticmethod
     def forward(ctx, u, delta, A, B, C, D, z, delta_bias, h0, delta_softplus, reverse):

@@ -163,6 +163,37 @@ def test_bf16_scan_op_checks():
                               test_utils=checks)
 
 
+@pytest.mark.parametrize("inside", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("leaf", [None, "A", "u"])
+def test_scan_of_tensors_without_memory(dtype, leaf, inside):
+    # what a trace sees, within the mode that made them and outside it
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    mode = FakeTensorMode()
+    inp = {k: mode.from_tensor(t.to(dtype) if t.dtype == torch.bfloat16 else t)
+           for k, t in bf16_scan(5)[0].items()}
+    if leaf:
+        inp[leaf].requires_grad_()
+
+    def run():
+        out, last = arm().selective_scan(**inp, delta_softplus=True, return_last_state=True)
+        if leaf:
+            (out.sum() + last.sum()).backward()
+        return out, last
+
+    if inside:
+        with mode:
+            out, last = run()
+    else:
+        out, last = run()
+    assert isinstance(out, FakeTensor) and out.dtype == last.dtype == torch.float32
+    assert out.shape == inp["u"].shape and last.shape == inp["initial_state"].shape
+    if leaf:
+        g = inp[leaf].grad
+        assert isinstance(g, FakeTensor) and g.shape == inp[leaf].shape
+        assert g.dtype == inp[leaf].dtype
+
+
 # ---------------------------------------------------------------------------
 # the patch in 16 bits
 def tiny_mamba(dtype=torch.float32):
